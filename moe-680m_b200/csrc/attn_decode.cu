@@ -12,7 +12,8 @@
 //   * the query heads of a group are the 16 rows of mma.sync.m16n8k16 tiles; a group of up to 8
 //     heads leaves 8 rows, which carry the second 16-bit piece of f32 queries and of the
 //     softmax weights, so both enter the products with twice a 16-bit type's precision at no cost
-//     (groups above 8 take a second product).  tcgen05 tiles have 128 rows: 120 of them would be empty;
+//     (groups above 8 take a second product): 22 bits (f16; weights times 2^15, so down to weights of 2^-18 of the
+//     largest, and below that to 2^-40 of it) or 16 (bf16).  tcgen05 tiles have 128 rows: 120 of them would be empty;
 //   * running maximum and sum per warp (f32, base 2); at the end of a sequence's part the warps hand
 //     theirs over through shared memory to 4 more warps and go on with their next units, while those join
 //     and store them (the copies never pause for it: 64 ragged sequences 181 -> 173 us);
@@ -115,6 +116,12 @@ attn_decode_kernel(const DecodeArgs p, const __grid_constant__ CUtensorMap kmap,
     constexpr int kKS = D / 16;                     // products per score tile
     constexpr int kNT = D / 8;                      // output tiles
     constexpr int kRows = WIDE ? 16 : 8;
+    // Weights e^(s - m) <= 1 enter the products times this.  An f16 piece below 2^-14 has the fewer bits the smaller it is
+    // (the last is 2^-24), and beside one key far above the rest all other weights are that small, while the
+    // total counts them in full: 8192 keys 18 below one whose value is zero, f32 result off by 9e-3 with weights times 1
+    // and by 4e-6 so; 24 below, 1.5e-2 and 1.5e-5 (times unchanged).  O and the totals carry the factor alike and it
+    // cancels.  bf16 has f32's range.
+    constexpr float kLift = std::is_same<C, __half>::value ? 32768.f : 1.f;
 
     extern __shared__ __align__(1024) uint8_t sm[];
     uint8_t* ring = sm;                                                   // [warp][stage]{K tile, V tile}
@@ -499,7 +506,7 @@ attn_decode_kernel(const DecodeArgs p, const __grid_constant__ CUtensorMap kmap,
                     float sum = 0.f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        z[r][i] = ex2(fmaf(z[r][i], sl[r], -base));
+                        z[r][i] = ex2(fmaf(z[r][i], sl[r], -base)) * kLift;
                         sum += z[r][i];
                     }
                     l[r] = fmaf(l[r], alpha[r], sum);
