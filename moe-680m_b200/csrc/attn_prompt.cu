@@ -17,9 +17,11 @@
 //     A operand of O += P V straight from TMEM; V is read as it lies in the page (MN-major), so nothing
 //     is transposed.  While one step's softmax runs, the tensor core works on another's products;
 //   * f32 queries enter as two 16-bit pieces (row scaled by a power of two for f16), and so do their
-//     weights: twice the products, 22-bit (bf16: 16-bit) precision;
-//   * O is rescaled only when a row's maximum has grown by more than 2^8 since the last time: until
-//     then its weights are up to 2^8, which the 16-bit types and the f32 sums hold as exactly.
+//     weights: twice the products, 22-bit (bf16: 16-bit) precision, for weights below 2^-16 of a row's largest
+//     (f16) to 2^-38 of that; 16-bit queries' weights are one piece of their type;
+//   * O is rescaled only when a row's maximum has grown by more than 2^8 (bf16) or 2^2 to 2^4 (f16, whose weights
+//     are lifted towards the type's largest value) since the last time: until then its weights are that much above
+//     1, which the 16-bit types and the f32 sums hold as exactly.
 // A key that a row does not see must not touch it whatever it holds.  Scores are replaced, but a weight of 0 times
 // an infinite or NaN value would be NaN; so in the tiles at the causal edge two warps put 0 in the place
 // of such values (and of all rows behind the sequence's end) before the product, keep for each
@@ -53,7 +55,19 @@ constexpr int kSoftmaxRegs = 184, kOtherRegs = 72;
 // sums are cut off, not rounded, at each of the products' additions (8192 keys, error of the output
 // against 64 bits: 6.2e-6 in one O, 1.9e-6 in parts of 16 steps, 1.2e-6 of 8; the time is the same).
 constexpr int kPart = 8;
-constexpr float kRescaleAt = 8.f;  // log2
+// Log2 of how far a row's maximum may grow before O is rescaled, and of a factor that the weights have on their way into
+// the products (O and the row's total carry it alike: it cancels).  An f16 piece below 2^-14 has the fewer bits the
+// smaller it is (the last is 2^-24), and beside one key far above the rest all other weights are that small.
+// Both together keep below f16's largest value, 2^15 in all.  8192 keys below one whose value is zero, error of an f32 result
+// and time of 8192 tokens:   factor 2^0    2^7     2^11    2^13    2^14
+//   18 below                  2.5e-1   5.2e-5  4.4e-6  3.8e-6  3.7e-6
+//   20 below                  8.7e-1   5.8e-4  2.2e-5  6.5e-6  5.0e-6
+//   f32 queries, D = 128      528 us   532     545     578     603
+//   f16 queries, D = 64       133 us   134     135     139     143     (packed ragged prompts)
+// f16 results have 11 bits and gain nothing from more than 2^11 (20 below: 4.7e-4 with 2^11 and 2^14).  bf16 has
+// f32's range.
+template <typename A, typename C> constexpr float kLift = std::is_same<C, __half>::value ? sizeof(A) == 4 ? 13.f : 11.f : 0.f;
+template <typename A, typename C> constexpr float kRescaleAt = std::is_same<C, __half>::value ? 15.f - kLift<A, C> : 8.f;
 struct PromptArgs {
     KvBatch b;
     AttnArgs a;
@@ -98,7 +112,7 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 }
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
-// 2^x for x <= 8 on the FMA pipes: x = n + f, |f| <= 1/2 (rounding by adding 1.5 * 2^23, whose low bits then
+// 2^x for x <= 16 on the FMA pipes: x = n + f, |f| <= 1/2 (rounding by adding 1.5 * 2^23, whose low bits then
 // hold n), 2^f = 1 + f p(f) with p the degree-4 interpolation of (2^f - 1) / f at the Chebyshev
 // points of [-1/2, 1/2] (relative error 2.6e-7), and n added to the exponent.  x <= -127 gives
 // exactly 0 (f = 0 there); NaN gives a value that no 16-bit type holds (infinite there).  One weight of 16
@@ -632,7 +646,7 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
                 mz = fmaxf(mz, theirs);
             }
             const float m_new = fmaxf(m, mz * sl);
-            const bool grown = __any_sync(0xffffffffu, m_new > m + kRescaleAt), part_end = kSplit && i0 > 0 && i0 % kPart == 0;
+            const bool grown = __any_sync(0xffffffffu, m_new > m + kRescaleAt<A, C>), part_end = kSplit && i0 > 0 && i0 % kPart == 0;
             if (grown || part_end) {
                 float f = 1.f;
                 if (grown) {
@@ -671,7 +685,7 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
             }
             const float base = m == -INFINITY ? 0.f : m;
             float2 sum[2] = {both(0.f), both(0.f)};
-            const float2 sl2 = both(sl), nb2 = both(-base);
+            const float2 sl2 = both(sl), nb2 = both(kLift<A, C> - base);
 #pragma unroll
             for (int c0 = kStep - kHeld; c0 >= 0; c0 -= kHeld) {
                 if (c0 + kHeld < kStep) take(c0);

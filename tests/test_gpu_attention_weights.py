@@ -3,8 +3,8 @@ looks at), through the C ABI against 64 bits.  The other keys' softmax weights a
 and make up the whole output where the first key's value is zero.
 
 Bound: the one of attention_ref.py, which takes a weight's rounding as relative to the weight, and beside it the smallest
-step of the 16-bit type that the weights enter the products in.  An f16 cache has the weights times 2^L (L = 15 in decode, 14
-in a prompt) as f16 pieces; the last piece is a multiple of 2^-24 and so off by at most 2^-25, which is
+step of the 16-bit type that the weights enter the products in.  An f16 cache has the weights times 2^L (L = 15 in decode, in a
+prompt 13 with f32 and 11 with f16 queries) as f16 pieces; the last piece is a multiple of 2^-24 and so off by at most 2^-25, which is
 2^-(25 + L) of the largest weight.  So each key adds at most 2^-(25 + L) |v| to the weighted sum's error, whose denominator is
 the sum of all weights over the largest.  The pieces of a bf16 cache have f32's range: nothing is added."""
 import pytest
@@ -16,7 +16,7 @@ from moe680m_b200 import host
 pytestmark = pytest.mark.gpu
 
 TYPES = [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")]
-LIFT = {"decode": 15, "prompt": 14}
+LIFT = {("decode", "f32"): 15, ("decode", "f16"): 15, ("prompt", "f32"): 13, ("prompt", "f16"): 11}
 
 
 @pytest.fixture
@@ -61,7 +61,7 @@ def check(b, kind, rows=None):
                 q = b.rows[t, :b.heads * b.dim].double().view(b.hkv, -1, b.dim)
                 s = torch.einsum("hgd,hkd->hgk", q, k[:, :keys]) * b.scale
                 total = (s - s.amax(-1, keepdim=True)).exp().sum(-1)
-                step = 2.0 ** -(25 + LIFT[kind]) / total[..., None] * v[:, :keys].abs().sum(1)[:, None]
+                step = 2.0 ** -(25 + LIFT[kind, b.act]) / total[..., None] * v[:, :keys].abs().sum(1)[:, None]
                 bound[t] += step.reshape(b.heads, b.dim)
     got = b.out()[:, :b.heads * b.dim].double().view_as(want)
     seen = torch.isfinite(want)
@@ -86,3 +86,28 @@ def test_decode_one_key_above_a_long_tail(ctx, gap):
     b = sink_batch(ctx, 52, [1], [262144], 2, 1, 64, 64, "f32", "f16", gap, [0], "both signs")
     b.decode()
     check(b, "decode")
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("gap", [10, 14, 17, 18, 20, 24])
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_one_key_above_the_rest(ctx, act, cache, gap, dim):
+    """The key at the front, in the middle and among the prompt's own; some rows do not see it yet."""
+    new, lens = [20, 40, 0, 37], [8192, 4100, 50, 127]
+    b = sink_batch(ctx, 53, new, lens, 4, 1, dim, 32, act, cache, gap, [0, 2900, 0, 100], "one sign")
+    b.prompt()
+    check(b, "prompt")
+
+
+@pytest.mark.parametrize("act,cache", TYPES)
+@pytest.mark.parametrize("dim", [64, 128])
+def test_prompt_maximum_that_grows_by_small_steps(ctx, act, cache, dim):
+    """Scores that climb by 1/4 of a unit every 64 keys to 20 and fall back: each step moves the maximum a little, and at the
+    end most weights are far below the largest."""
+    n = 8192
+    b = sink_batch(ctx, 54, [16], [n], 4, 1, dim, 64, act, cache, 0, [0], "one sign")
+    for i in range(0, n, 64):
+        b.k[0, b.table[0, i // 64], :, :, 0] = min(i // 64, 80) * 0.25 * 4 if i < n // 2 else -40.0
+    ctx.upload(b.k_off, raw(b.k))
+    b.prompt()
+    check(b, "prompt")
