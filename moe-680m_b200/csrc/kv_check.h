@@ -64,6 +64,7 @@ inline int kv_check_spec(const KvSpec& s, uint64_t arena, std::string* err) {
 // Bytes of `rows` rows of `width` values, `stride` values apart; 0 when a number is out of range.
 inline uint64_t kv_rows_bytes(uint64_t rows, uint64_t stride, uint64_t width, uint64_t size) {
     if (stride < width || stride > (1ull << 40) || rows == 0) return 0;
+    if (stride && rows - 1 > (~0ull / size - width) / stride) return 0;  // past 64 bits
     return ((rows - 1) * stride + width) * size;
 }
 
@@ -84,7 +85,7 @@ inline int kv_check_call(const KvSpec& s, const KvCall& c, uint64_t arena, bool 
     const uint64_t size = kv_type_bytes(c.type), per16 = 16 / size;
     const uint64_t na = kv_rows_bytes(c.tokens, c.a_stride, c.a_width, size), nb = kv_rows_bytes(c.tokens, c.b_stride, c.b_width, size);
     if (na == 0 || nb == 0 || c.a_stride % per16 || c.b_stride % per16)
-        return kv_refuse(err, MOE_E_INVALID, "row stride below the row's width, or not a multiple of 16 bytes");
+        return kv_refuse(err, MOE_E_INVALID, "row stride below the row's width or too large, or not a multiple of 16 bytes");
     if (!kv_in_arena(arena, c.a_off, na, 16) || !kv_in_arena(arena, c.b_off, nb, 16))
         return kv_refuse(err, MOE_E_INVALID, "rows outside the arena or not 16-byte aligned");
     const uint64_t pool = s.pool_bytes();
