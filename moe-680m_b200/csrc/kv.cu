@@ -19,8 +19,10 @@ namespace {
 template <typename A, typename C>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvBatch b, const A* __restrict__ k, const A* __restrict__ v,
                                                         uint64_t stride, int T, C* __restrict__ kp, C* __restrict__ vp) {
-    const int t = static_cast<int>((blockIdx.x * 256u + threadIdx.x) >> 5), lane = threadIdx.x & 31;
-    if (t >= T) return;
+    // a batch has up to 2^31 - 1 tokens: the token's number, not its thread's, fits 32 bits
+    const unsigned token = blockIdx.x * 8u + threadIdx.x / 32u;
+    if (token >= static_cast<unsigned>(T)) return;
+    const int t = static_cast<int>(token), lane = threadIdx.x & 31;
     const int s = warp_seq_of_token(b, t, lane);
     if (s < 0) return;
     const int n_after = b.cu ? b.cu[s + 1] - t : 1;  // tokens from this one to its sequence's end
@@ -61,7 +63,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvBatch b, const A
 
 template <typename A, typename C>
 void append_t(const KvBatch& b, const void* k, const void* v, uint64_t stride, int T, void* kp, void* vp, cudaStream_t s) {
-    kv_append_kernel<A, C><<<static_cast<unsigned>((T + 7) / 8), 256, 0, s>>>(
+    kv_append_kernel<A, C><<<(static_cast<unsigned>(T) + 7) / 8, 256, 0, s>>>(
         b, static_cast<const A*>(k), static_cast<const A*>(v), stride, T, static_cast<C*>(kp), static_cast<C*>(vp));
 }
 

@@ -75,6 +75,7 @@ inline int kv_check_call(const KvSpec& s, const KvCall& c, uint64_t arena, bool 
     if (c.type != MOE_T_F32 && c.type != s.type)
         return kv_refuse(err, MOE_E_UNSUPPORTED, "16-bit activations of another type than the cache's");
     if (c.n_seqs > kMaxBatchSeqs) return kv_refuse(err, MOE_E_UNSUPPORTED, "n_seqs " + std::to_string(c.n_seqs) + ": at most 4096");
+    if (c.tokens > 0x7FFFFFFFu) return kv_refuse(err, MOE_E_UNSUPPORTED, "2^31 tokens or more");  // offsets have 31 bits
     if (c.cu_off == 0 && c.tokens != c.n_seqs)
         return kv_refuse(err, MOE_E_INVALID, "without offsets there is one token for each sequence");
     if (c.max_pages == 0 || static_cast<uint64_t>(c.max_pages) * s.page_size > 2147483392ull)

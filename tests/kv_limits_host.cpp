@@ -51,8 +51,25 @@ static void rows_past_64_bits() {
     EXPECT(moe::kv_check_call(s, c, arena, true, &err) == MOE_OK);
 }
 
+// Offsets of packed tokens have 31 bits.
+static void token_numbers() {
+    const uint64_t arena = 1ull << 50;
+    moe::KvSpec s;
+    s.type = MOE_T_F16; s.n_layers = 1; s.n_kv_heads = 1; s.head_dim = 64; s.page_size = 16; s.n_pages = 8;
+    s.k_off = 256; s.v_off = 256 + s.pool_bytes();
+    moe::KvCall c;
+    const uint64_t top = s.v_off + s.pool_bytes();
+    c.type = MOE_T_F16; c.n_seqs = 1; c.max_pages = 4; c.cu_off = top; c.table_off = top + 256; c.lens_off = top + 512;
+    c.a_off = top + 1024; c.b_off = 1ull << 45; c.a_width = c.b_width = 64; c.a_stride = c.b_stride = 64;
+    for (const uint32_t n : {1u, 0x7FFFFFFFu, 0x80000000u, 0xFFFFFFFFu}) {
+        c.tokens = n;
+        for (const bool write : {true, false}) EXPECT(moe::kv_check_call(s, c, arena, write, &err) == (n >> 31 ? MOE_E_UNSUPPORTED : MOE_OK));
+    }
+}
+
 int main() {
     rows_past_64_bits();
+    token_numbers();
     std::puts("kv limits ok");
     return 0;
 }
