@@ -353,8 +353,9 @@ int moe_silu_mul(moe_ctx* ctx, uint64_t g_off, uint64_t u_off, uint64_t y_off, u
  * i32 [n_seqs] at lens_off, and, for packed tokens, offsets i32 [n_seqs + 1] at cu_off: sequence s has the packed
  * rows [cu[s], cu[s+1]) of `tokens` rows; they are the last of its lens[s] tokens (the length counts
  * them).  cu_off 0: one token for each sequence (tokens == n_seqs).  Rows behind cu[n_seqs] are not read
- * or written.  A page id outside the cache, a length outside its table row or an appended token in
- * front of its sequence makes moe_sync return MOE_E_DEVICE; nothing outside the arena's tensors is touched.
+ * or written.  A page id outside the cache, a length outside its table row, offsets that do not ascend or
+ * leave the rows (such a sequence counts as one without tokens), or an appended token in front of its sequence
+ * makes moe_sync return MOE_E_DEVICE; nothing outside the arena's tensors is touched.
  *
  * Types: rows are f32, or 16-bit of the cache's type; strides are counted in values; offsets and
  * strides are multiples of 16 bytes.  All sums and softmax statistics are f32. */

@@ -19,13 +19,25 @@ namespace {
 template <typename A, typename C>
 __global__ void __launch_bounds__(256) kv_append_kernel(const KvBatch b, const A* __restrict__ k, const A* __restrict__ v,
                                                         uint64_t stride, int T, C* __restrict__ kp, C* __restrict__ vp) {
+    if (blockIdx.x == gridDim.x - 1 && b.cu) {
+        // A block more than the tokens take, off their path: offsets that do not ascend or that leave the rows.  (A
+        // token's own search meets only some of them.)
+        for (int i = threadIdx.x; i < b.n_seqs; i += 256)
+            if (!right_offsets(b.cu[i], b.cu[i + 1], T)) set_dev_error(b.status, kDevBadToken);
+        return;
+    }
     // a batch has up to 2^31 - 1 tokens: the token's number, not its thread's, fits 32 bits
     const unsigned token = blockIdx.x * 8u + threadIdx.x / 32u;
     if (token >= static_cast<unsigned>(T)) return;
     const int t = static_cast<int>(token), lane = threadIdx.x & 31;
     const int s = warp_seq_of_token(b, t, lane);
     if (s < 0) return;
-    const int n_after = b.cu ? b.cu[s + 1] - t : 1;  // tokens from this one to its sequence's end
+    const int from = b.cu ? b.cu[s] : t, to = b.cu ? b.cu[s + 1] : t + 1;
+    if (!right_offsets(from, to, T) || t < from || t >= to) {
+        set_dev_error(b.status, kDevBadToken);
+        return;
+    }
+    const int n_after = to - t;  // tokens from this one to its sequence's end
     const long long pos = static_cast<long long>(b.lens[s]) - n_after;
     if (pos < 0 || pos >= static_cast<long long>(b.max_pages) * b.page_size) {
         set_dev_error(b.status, kDevBadToken);
@@ -63,7 +75,7 @@ __global__ void __launch_bounds__(256) kv_append_kernel(const KvBatch b, const A
 
 template <typename A, typename C>
 void append_t(const KvBatch& b, const void* k, const void* v, uint64_t stride, int T, void* kp, void* vp, cudaStream_t s) {
-    kv_append_kernel<A, C><<<(static_cast<unsigned>(T) + 7) / 8, 256, 0, s>>>(
+    kv_append_kernel<A, C><<<(static_cast<unsigned>(T) + 7) / 8 + (b.cu ? 1 : 0), 256, 0, s>>>(
         b, static_cast<const A*>(k), static_cast<const A*>(v), stride, T, static_cast<C*>(kp), static_cast<C*>(vp));
 }
 

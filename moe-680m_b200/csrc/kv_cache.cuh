@@ -82,6 +82,9 @@ __device__ __forceinline__ int checked_len(int len, const KvBatch& b, int* statu
     return len < 0 ? 0 : static_cast<int>(cap);
 }
 
+// Whether a sequence can have the packed rows [from, to) of T.
+__device__ __forceinline__ bool right_offsets(int from, int to, int T) { return from >= 0 && from <= to && to <= T; }
+
 // The sequence whose packed tokens [cu[s], cu[s+1]) hold token t, or -1 behind the last one (and
 // in front of the first); without offsets every sequence has one token.  By a whole warp: 32 offsets at a
 // time, so that up to 31 sequences take one round of loads.
