@@ -218,8 +218,8 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
     // a sequence's packed tokens; wrong offsets are reported and count as none
     auto tokens_of = [&](int s, int* t0) {
         *t0 = b.cu ? b.cu[s] : s;
-        const int n = (b.cu ? b.cu[s + 1] : s + 1) - *t0;
-        if (*t0 >= 0 && n >= 0 && *t0 <= p.a.T - n) return n;
+        const int end = b.cu ? b.cu[s + 1] : s + 1;
+        if (right_offsets(*t0, end, p.a.T)) return end - *t0;
         set_dev_error(b.status, kDevBadToken);
         return 0;
     };
@@ -281,7 +281,7 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
                 sh->n_new = n;
             }
             __syncthreads();
-            if (target < carry) break;
+            if (target < carry && target > 0) break;  // the first unit's blocks look over all offsets
         }
         if (sh->seq < 0) return;
         seq = uniform(sh->seq);
