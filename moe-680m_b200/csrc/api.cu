@@ -1799,8 +1799,7 @@ int moe_kv_seq_fork(moe_ctx* c, uint32_t kv_id, const uint64_t* parents, uint32_
     if (stream_capturing(c)) return fail(c, MOE_E_INVALID, "moe_kv_seq_fork cannot be captured");
     return kv_guarded(c, [&] {
         moe::KvPages::Moves copies;
-        const int r = kv->pages.fork(parents, n, children, &copies, &c->err);
-        return r ? r : kv_run_copies(c, kv->spec, copies);
+        return kv->pages.fork(parents, n, children, &copies, &c->err, [&](const auto& m) { return kv_run_copies(c, kv->spec, m); });
     });
 }
 
@@ -1820,9 +1819,9 @@ int moe_kv_compact(moe_ctx* c, uint32_t kv_id, uint64_t* n_moved) {
     if (stream_capturing(c)) return fail(c, MOE_E_INVALID, "moe_kv_compact cannot be captured");
     return kv_guarded(c, [&] {
         moe::KvPages::Moves moves;
-        kv->pages.compact(&moves);
-        if (n_moved) *n_moved = moves.size();
-        return kv_run_copies(c, kv->spec, moves);
+        const int r = kv->pages.compact(&moves, [&](const auto& m) { return kv_run_copies(c, kv->spec, m); });
+        if (!r && n_moved) *n_moved = moves.size();
+        return r;
     });
 }
 

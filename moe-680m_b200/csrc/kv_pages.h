@@ -23,6 +23,7 @@ namespace moe {
 class KvPages {
 public:
     using Moves = std::vector<std::pair<uint32_t, uint32_t>>;  // (from, to) pages
+    using Copy = std::function<int(const Moves&)>;             // makes the copies on the device: MOE_OK or an error
 
     KvPages(uint32_t n_pages, uint32_t page_size) : page_size_(page_size), users_(n_pages, 0) {
         std::vector<uint32_t> all(n_pages);
@@ -77,8 +78,8 @@ public:
     }
 
     // One child per parent (a parent may be given more than once): full pages are shared, a partly
-    // filled last page gets a page of its own, listed in `copies`.
-    int fork(const uint64_t* parents, uint32_t n, uint64_t* children, Moves* copies, std::string* err) {
+    // filled last page gets a page of its own, listed in `copies` and copied by `copy`.
+    int fork(const uint64_t* parents, uint32_t n, uint64_t* children, Moves* copies, std::string* err, const Copy& copy = nullptr) {
         int rc = check(parents, n, true, err);
         if (rc) return rc;
         uint64_t need = 0;
@@ -100,8 +101,20 @@ public:
                 copies->emplace_back(child.pages.back(), p);
                 child.pages.back() = p;
             }
-            children[i] = made[i];
         }
+        if (copy) {
+            try {
+                rc = copy(*copies);
+            } catch (...) {
+                free(made.data(), n, err);
+                throw;
+            }
+            if (rc) {
+                free(made.data(), n, err);  // of living sequences, each once: it cannot fail
+                return rc;
+            }
+        }
+        for (uint32_t i = 0; i < n; ++i) children[i] = made[i];
         return MOE_OK;
     }
 
@@ -122,26 +135,29 @@ public:
     }
 
     // Moves the used pages into ids [0, used): the i-th used page at or above that bound goes to the
-    // i-th free page below it, so no page is both read and written.
-    void compact(Moves* moves) {
+    // i-th free page below it, so no page is both read and written.  The copies are made (`copy`) before anything changes:
+    // they write free pages only.
+    int compact(Moves* moves, const Copy& copy = nullptr) {
         const uint32_t used = n_pages() - n_free();
-        std::vector<uint32_t> to(users_.size());
+        std::vector<uint32_t> to(users_.size()), rest;
         for (uint32_t p = 0; p < to.size(); ++p) to[p] = p;
         moves->reserve(used);
+        rest.reserve(users_.size());  // the heap never grows past it
         uint32_t hole = 0;
         for (uint32_t p = used; p < users_.size(); ++p) {
+            rest.push_back(p);
             if (users_[p] == 0) continue;
             while (users_[hole] != 0) ++hole;
             moves->emplace_back(p, hole);
             to[p] = hole++;
         }
+        if (copy)
+            if (const int rc = copy(*moves)) return rc;
         for (const auto& m : *moves) std::swap(users_[m.first], users_[m.second]);
         for (Seq& s : seqs_)
             for (uint32_t& p : s.pages) p = to[p];
-        std::vector<uint32_t> rest;
-        rest.reserve(users_.size());
-        for (uint32_t p = used; p < users_.size(); ++p) rest.push_back(p);
         free_ = Heap(std::greater<uint32_t>(), std::move(rest));
+        return MOE_OK;
     }
 
     // The table rows of n sequences ([n][max_pages], unused entries 0), then their n lengths.
