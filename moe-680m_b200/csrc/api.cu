@@ -1919,8 +1919,6 @@ static int run_attn(Ctx* c, uint32_t kv_id, bool decode, uint32_t layer, uint32_
         DeviceGuard g(c->device);
         moe::AttnArgs a{};
         a.q = c->base + q_off; a.out = c->base + out_off; a.q_stride = q_stride; a.out_stride = out_stride;
-        a.k = c->base + s.k_off + layer * s.layer_bytes();
-        a.v = c->base + s.v_off + layer * s.layer_bytes();
         a.n_heads = static_cast<int>(n_heads); a.T = static_cast<int>(tokens); a.scale = scale;
         if (decode)
             moe::launch_attn_decode(kv_batch(c, s, call), static_cast<int>(type), *kv, layer, a, c->attn_ws, c->sm_count, c->stream);

@@ -277,7 +277,9 @@ attn_decode_kernel(const DecodeArgs p, const __grid_constant__ CUtensorMap kmap,
                         for (int i = 0; i < 16; ++i)
 #pragma unroll
                             for (int d = 0; d < D / 64; ++d)
-                                x[i][d] = there && i0 + i < n ? __ldcg(reinterpret_cast<const float4*>(p.part_o + slot_of(c + (i0 + i) * step, row) * D + k * 4 + 64 * d)) : make_float4(0.f, 0.f, 0.f, 0.f);
+                                x[i][d] = there && i0 + i < n
+                                              ? __ldcg(reinterpret_cast<const float4*>(p.part_o + slot_of(c + (i0 + i) * step, row) * D + k * 4 + 64 * d))
+                                              : make_float4(0.f, 0.f, 0.f, 0.f);
                         float mx = fmaxf(m_all, ml.x);
 #pragma unroll
                         for (int o = 8; o > 0; o >>= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
@@ -405,7 +407,7 @@ attn_decode_kernel(const DecodeArgs p, const __grid_constant__ CUtensorMap kmap,
                 for (int k = 0; k < kKS; ++k)
 #pragma unroll
                     for (int i = 0; i < 4; ++i) qf[r][k][i] = row < n_rows ? to_f32(q[16 * k + 8 * (i >> 1) + (i & 1)]) : 0.f;
-                if constexpr (kSplitQ && sizeof(C) == 2) {
+                if constexpr (kSplitQ) {
                     if constexpr (std::is_same<C, __half>::value) {
                         // f16 pieces: the row's largest magnitude goes to [2^14, 2^15), undone in its score scale
                         float mx = 0.f;
@@ -453,7 +455,8 @@ attn_decode_kernel(const DecodeArgs p, const __grid_constant__ CUtensorMap kmap,
                     for (int i = lane; i < kTile * (D / 8); i += 32) {
                         const int row = i / (D / 8), c = i % (D / 8);
                         if (t0 + row >= len)
-                            *reinterpret_cast<uint4*>(v + (row / kBoxRows) * kBoxBytes + (c >> 3) * (kBoxRows * 128) + (row % kBoxRows) * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
+                            *reinterpret_cast<uint4*>(v + (row / kBoxRows) * kBoxBytes + (c >> 3) * (kBoxRows * 128) +
+                                                      (row % kBoxRows) * 128 + ((c & 7) << 4)) = make_uint4(0, 0, 0, 0);
                     }
                     tc::fence_proxy_async_smem();  // ordered before the copy that reuses the slot
                     __syncwarp();

@@ -376,7 +376,9 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
                 for (int h = 0; h < kPieces; ++h)
 #pragma unroll
                     for (int k = 0; k < kStep / 16; ++k)
-                        if (k < ksteps) tc::mma_ts(o_at, s_at + (i % kSBufs) * kStep + kPCol + h * 32 + k * 8, v_at + k * (2048 >> 4), idesc_o, ((kSplit ? i % kPart : i) | h | k) != 0);
+                        if (k < ksteps)
+                            tc::mma_ts(o_at, s_at + (i % kSBufs) * kStep + kPCol + h * 32 + k * 8, v_at + k * (2048 >> 4), idesc_o,
+                                       ((kSplit ? i % kPart : i) | h | k) != 0);
                 if ((i & 1) || i + 1 == n) tc::mma_commit(&sh->kv_empty[vbuf]);
             };
             auto wait_k = [&](int j) { return wait(&sh->kv_full[2 * j % kBufs], (2 * j / kBufs) & 1, sh); };
@@ -534,61 +536,57 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
                 }
                 asm volatile("cp.async.wait_all;" ::: "memory");
             } else {
-            constexpr int kSteps = 32 / kRowsPer / kPer, kBatch = kSteps < 8 ? kSteps : 8;  // a group's share of the rows
-            uint4 in[kBatch], ahead[kBatch];  // a batch of rows is loaded while the one before is worked on
-            auto load = [&](int i0, uint4 (&to)[kBatch]) {
+                constexpr int kSteps = 32 / kRowsPer / kPer, kBatch = kSteps < 8 ? kSteps : 8;  // a group's share of the rows
+                uint4 in[kBatch], ahead[kBatch];  // a batch of rows is loaded while the one before is worked on
+                auto load = [&](int i0, uint4 (&to)[kBatch]) {
 #pragma unroll
-                for (int k = 0; k < kBatch; ++k) {
-                    const int src = (g * kSteps + i0 + k) * kRowsPer + lane / kLanesPer;  // row of the warp
-                    const size_t off = __shfl_sync(0xffffffffu, q_off, src);
-                    const bool there = __shfl_sync(0xffffffffu, live, src);
-                    to[k] = there ? __ldg(reinterpret_cast<const uint4*>(static_cast<const A*>(p.a.q) + off) + part) : make_uint4(0, 0, 0, 0);
-                }
-            };
-            load(0, ahead);
-#pragma unroll 1
-            for (int i0 = 0; i0 < kSteps; i0 += kBatch) {
-#pragma unroll
-            for (int k = 0; k < kBatch; ++k) in[k] = ahead[k];
-            if (i0 + kBatch < kSteps) load(i0 + kBatch, ahead);
-#pragma unroll
-            for (int k0 = 0; k0 < kBatch; ++k0) {
-                const int i = (g * kSteps + i0 + k0) * kRowsPer, src = i + lane / kLanesPer;
-                alignas(16) A x[kVals];
-                *reinterpret_cast<uint4*>(x) = in[k0];
-                const int rr = (warp & 3) * 32 + src;
-                const int c = part * kVals / 8;  // 16-byte chunk of 16-bit values
-                uint8_t* at = qs + t * kPieces * kTileBytes + (c >> 3) * kHalfBytes + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
-                if constexpr (kSplit) {
-                    float f[4] = {to_f32(x[0]), to_f32(x[1]), to_f32(x[2]), to_f32(x[3])};
-                    if constexpr (kHalfType) {
-                        // the row's largest magnitude goes to [2^14, 2^15), undone in its score scale
-                        float mx = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
-                        if constexpr (kLanesPer == 32) {  // magnitudes order as their bits do
-                            mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
-                        } else {
-#pragma unroll
-                            for (int o = 1; o < kLanesPer; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
-                        }
-                        const int e = row_exponent(mx);
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) f[k] *= pow2(e);
-#pragma unroll
-                        for (int k = 0; k < kRowsPer; ++k) {
-                            const int ek = __shfl_sync(0xffffffffu, e, k * kLanesPer);
-                            if (lane == i + k) sl *= pow2(-ek);
-                        }
+                    for (int k = 0; k < kBatch; ++k) {
+                        const int src = (g * kSteps + i0 + k) * kRowsPer + lane / kLanesPer;  // row of the warp
+                        const size_t off = __shfl_sync(0xffffffffu, q_off, src);
+                        const bool there = __shfl_sync(0xffffffffu, live, src);
+                        to[k] = there ? __ldg(reinterpret_cast<const uint4*>(static_cast<const A*>(p.a.q) + off) + part) : make_uint4(0, 0, 0, 0);
                     }
-                    uint2 hi, lo;
-                    hi.x = pack2<C>(f[0], f[1]); hi.y = pack2<C>(f[2], f[3]);
-                    lo.x = pack_rest<C>(hi.x, f[0], f[1]); lo.y = pack_rest<C>(hi.y, f[2], f[3]);
-                    *reinterpret_cast<uint2*>(at + (part & 1) * 8) = hi;
-                    *reinterpret_cast<uint2*>(at + kTileBytes + (part & 1) * 8) = lo;
-                } else {
-                    *reinterpret_cast<uint4*>(at) = *reinterpret_cast<uint4*>(x);
+                };
+                load(0, ahead);
+#pragma unroll 1
+                for (int i0 = 0; i0 < kSteps; i0 += kBatch) {
+#pragma unroll
+                    for (int k = 0; k < kBatch; ++k) in[k] = ahead[k];
+                    if (i0 + kBatch < kSteps) load(i0 + kBatch, ahead);
+#pragma unroll
+                    for (int k0 = 0; k0 < kBatch; ++k0) {
+                        const int i = (g * kSteps + i0 + k0) * kRowsPer, src = i + lane / kLanesPer;
+                        alignas(16) A x[kVals];
+                        *reinterpret_cast<uint4*>(x) = in[k0];
+                        const int rr = (warp & 3) * 32 + src;
+                        const int c = part * kVals / 8;  // 16-byte chunk of 16-bit values
+                        uint8_t* at = qs + t * kPieces * kTileBytes + (c >> 3) * kHalfBytes + rr * 128 + (((c & 7) ^ (rr & 7)) << 4);
+                        float f[4] = {to_f32(x[0]), to_f32(x[1]), to_f32(x[2]), to_f32(x[3])};
+                        if constexpr (kHalfType) {
+                            // the row's largest magnitude goes to [2^14, 2^15), undone in its score scale
+                            float mx = fmaxf(fmaxf(fabsf(f[0]), fabsf(f[1])), fmaxf(fabsf(f[2]), fabsf(f[3])));
+                            if constexpr (kLanesPer == 32) {  // magnitudes order as their bits do
+                                mx = __uint_as_float(__reduce_max_sync(0xffffffffu, __float_as_uint(mx)));
+                            } else {
+#pragma unroll
+                                for (int o = 1; o < kLanesPer; o <<= 1) mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, o));
+                            }
+                            const int e = row_exponent(mx);
+#pragma unroll
+                            for (int k = 0; k < 4; ++k) f[k] *= pow2(e);
+#pragma unroll
+                            for (int k = 0; k < kRowsPer; ++k) {
+                                const int ek = __shfl_sync(0xffffffffu, e, k * kLanesPer);
+                                if (lane == i + k) sl *= pow2(-ek);
+                            }
+                        }
+                        uint2 hi, lo;
+                        hi.x = pack2<C>(f[0], f[1]); hi.y = pack2<C>(f[2], f[3]);
+                        lo.x = pack_rest<C>(hi.x, f[0], f[1]); lo.y = pack_rest<C>(hi.y, f[2], f[3]);
+                        *reinterpret_cast<uint2*>(at + (part & 1) * 8) = hi;
+                        *reinterpret_cast<uint2*>(at + kTileBytes + (part & 1) * 8) = lo;
+                    }
                 }
-            }
-            }
             }
             tc::fence_proxy_async_smem();
             __syncwarp();
@@ -795,7 +793,8 @@ void launch_t(const PromptArgs& p, const CUtensorMap& k, const CUtensorMap& v, c
         cudaFuncSetAttribute(attn_prompt_kernel<A, C, D>, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(kSmem));
         if (dev < 64) set.fetch_or(1ull << dev);
     }
-    attn_prompt_kernel<A, C, D><<<static_cast<unsigned>(units_of(p.b, p.a, p.group, p.unit_rows)), Roles<kTiles, kSlimOf<A, D>>::kThreads, kSmem, s>>>(p, k, v);
+    const unsigned grid = static_cast<unsigned>(units_of(p.b, p.a, p.group, p.unit_rows));
+    attn_prompt_kernel<A, C, D><<<grid, Roles<kTiles, kSlimOf<A, D>>::kThreads, kSmem, s>>>(p, k, v);
 }
 
 template <typename A, typename C>

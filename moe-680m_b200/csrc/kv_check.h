@@ -119,7 +119,8 @@ inline int kv_check_tables(const KvSpec& s, uint64_t arena, uint32_t n, uint32_t
 
 inline int kv_check_heads(const KvSpec& s, const KvCall& c, uint32_t n_heads, float scale, std::string* err) {
     if (n_heads == 0 || n_heads > 4096 || n_heads % s.n_kv_heads != 0)
-        return kv_refuse(err, MOE_E_INVALID, "n_heads " + std::to_string(n_heads) + ": a multiple of the cache's " + std::to_string(s.n_kv_heads) + ", at most 4096");
+        return kv_refuse(err, MOE_E_INVALID, "n_heads " + std::to_string(n_heads) + ": a multiple of the cache's " +
+                                                 std::to_string(s.n_kv_heads) + ", at most 4096");
     if (static_cast<uint64_t>(c.tokens) * n_heads > 0x7FFFFFFFull / 2) return kv_refuse(err, MOE_E_UNSUPPORTED, "2^30 query rows or more");
     if (!(scale > 0.f) || !std::isfinite(scale)) return kv_refuse(err, MOE_E_INVALID, "scale must be positive and finite");
     return MOE_OK;

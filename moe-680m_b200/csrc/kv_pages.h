@@ -168,7 +168,8 @@ public:
         for (uint32_t i = 0; i < n; ++i) {
             const Seq& s = at(h[i]);
             if (s.pages.size() > max_pages)
-                return fail(err, MOE_E_INVALID, "sequence " + std::to_string(i) + " has " + std::to_string(s.pages.size()) + " pages, the table rows " + std::to_string(max_pages));
+                return fail(err, MOE_E_INVALID, "sequence " + std::to_string(i) + " has " + std::to_string(s.pages.size()) +
+                                                    " pages, the table rows " + std::to_string(max_pages));
             for (size_t j = 0; j < s.pages.size(); ++j) (*out)[static_cast<size_t>(i) * max_pages + j] = static_cast<int32_t>(s.pages[j]);
             (*out)[static_cast<size_t>(n) * max_pages + i] = static_cast<int32_t>(s.len);
         }

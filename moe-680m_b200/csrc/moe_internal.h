@@ -302,8 +302,6 @@ struct AttnArgs {
     const void* q;
     void* out;
     uint64_t q_stride, out_stride;  // values between token rows
-    const void* k;                  // the layer's pools
-    const void* v;
     int n_heads, T;
     float scale;
 };
