@@ -358,7 +358,16 @@ int moe_silu_mul(moe_ctx* ctx, uint64_t g_off, uint64_t u_off, uint64_t y_off, u
  * makes moe_sync return MOE_E_DEVICE; nothing outside the arena's tensors is touched.
  *
  * Types: rows are f32, or 16-bit of the cache's type; strides are counted in values; offsets and
- * strides are multiples of 16 bytes.  All sums and softmax statistics are f32. */
+ * strides are multiples of 16 bytes.  All sums and softmax statistics are f32.
+ *
+ * Precision of attention: products take operands of the cache's type.  f32 queries enter as two such pieces
+ * (22 bits with an f16 cache, 16 with bf16), and so do softmax weights in decode and with f32 queries; with 16-bit
+ * queries a prompt's weights are one piece (11 bits f16, 8 bf16: errors of the size of the outputs' own rounding).
+ * With an f16 cache, whose smallest step is fixed, small weights have fewer bits: beside the above a weight is off by
+ * up to 2^-36 (prompt, f16 queries), 2^-38 (prompt, f32) or 2^-40 (decode) of its row's largest.
+ * NaN and infinity: a row whose query or whose visible keys give a NaN score is NaN.  An infinite or NaN value makes its
+ * column not finite in the rows that see it, NaN where the definition may be infinite (a weight's second piece
+ * times infinity is NaN), and touches no other row. */
 #define MOE_T_F32 0u
 #define MOE_T_F16 1u
 #define MOE_T_BF16 2u
@@ -367,14 +376,14 @@ int moe_silu_mul(moe_ctx* ctx, uint64_t g_off, uint64_t u_off, uint64_t y_off, u
 uint64_t moe_kv_pool_bytes(uint32_t n_layers, uint32_t n_kv_heads, uint32_t head_dim, uint32_t page_size,
                            uint32_t n_pages);
 /* A cache over the pools at k_off and v_off (256-byte aligned, contents kept).  type MOE_T_F16 or MOE_T_BF16,
- * head_dim 64 or 128, page_size 16, 32, 64 or 128.  Returns an id >= 0, valid until the context is
+ * head_dim 64 or 128, page_size 16, 32, 64 or 128.  *kv_id gets its id, valid until the context is
  * destroyed. */
 int moe_kv_create(moe_ctx* ctx, uint32_t type, uint32_t n_layers, uint32_t n_kv_heads, uint32_t head_dim,
                   uint32_t page_size, uint32_t n_pages, uint64_t k_off, uint64_t v_off, uint32_t* kv_id);
 
 /* Sequences.  Handles are never 0 and not valid after moe_kv_seq_free.  Each call does all of its work or, with
  * an error, none: MOE_E_INVALID for a handle of no living sequence or one given twice, MOE_E_OOM when
- * too few pages are free.  Pages are handed out lowest free id first, and a freed page at once: work on
+ * too few pages or too little host memory are free, MOE_E_CUDA when page copies cannot be launched.  Pages are handed out lowest free id first, and a freed page at once: work on
  * another stream that still reads it has to be ordered by the caller.  Creating a cache, forking, compacting
  * and uploading tables are refused during stream capture. */
 int moe_kv_seq_create(moe_ctx* ctx, uint32_t kv_id, uint32_t n, uint64_t* seqs);
@@ -407,8 +416,9 @@ int moe_kv_append(moe_ctx* ctx, uint32_t kv_id, uint32_t layer, uint32_t type, u
  * p of its sequence (head h, kv head h / (n_heads / n_kv_heads)) gives
  *   out = sum_{t <= p} w_t v_t,  w = softmax_t(scale * q . k_t),
  * the tokens of an earlier part of the prompt included.  A row without a visible token (an empty sequence,
- * or more new tokens than the length counts) gives zeros; stored rows behind a sequence's length never count, whatever they hold.  q rows and out rows are
- * [n_heads][head_dim]; out must overlap neither q, the cache nor the table, lengths and offsets.  The same call gives the same bits. */
+ * or more new tokens than the length counts) gives zeros; stored rows behind a sequence's length never count,
+ * whatever they hold.  q rows and out rows are [n_heads][head_dim]; out must overlap neither q, the cache nor the
+ * table, lengths and offsets.  The same call gives the same bits. */
 int moe_attn_prompt(moe_ctx* ctx, uint32_t kv_id, uint32_t layer, uint32_t type, uint64_t q_off, uint64_t q_stride,
                     uint32_t n_heads, uint32_t n_seqs, uint64_t cu_off, uint32_t tokens, uint64_t table_off,
                     uint32_t max_pages, uint64_t lens_off, float scale, uint64_t out_off, uint64_t out_stride);

@@ -141,11 +141,11 @@ __device__ __forceinline__ bool wait(uint64_t* bar, uint32_t parity, Shared* sh)
 }
 
 // f32 queries of 128 columns take one row tile per CTA: with two, TMEM has no room for a second O (8192
-// tokens: 455 us so, with an error of 6.2e-6; 521 us and 1.2e-6 with one).
+// tokens, weights not lifted: 455 us so, with an error of 6.2e-6; 521 us and 1.2e-6 with one).
 template <typename A, int D> constexpr int kTilesOf = sizeof(A) == 4 && D == 128 ? 1 : 2;
 // 16-bit queries of 64 columns: their CTAs take half of an SM's TMEM, registers and shared memory, so two run at
-// once, with one place for S to each tile (9 ragged prompts up to 2500 tokens, 7 heads to a kv head: 147 us as
-// one CTA with two places, 132 so).
+// once, with one place for S to each tile (9 ragged prompts up to 2500 tokens, 7 heads to a kv head, weights not
+// lifted: 147 us as one CTA with two places, 132 so).
 template <typename A, int D> constexpr bool kSlimOf = sizeof(A) == 2 && D == 64;
 template <typename A, int D> constexpr int kBufsOf = kSlimOf<A, D> ? 4 : D == 64 ? 8 : 5;
 
@@ -168,7 +168,7 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
     // 48 clocks, for 32 of arithmetic; 8192 tokens, bf16: 80 % busy, 66 % computing), but 128 need both steps' places at
     // once, and with two tiles nothing is then ahead of the softmax (250 us with 64, 282 with 128).  A single tile has
     // four places, so S of two steps goes at once, and two threads take a row, one for each step (8192
-    // tokens, f32: 527 us with a step at a time and a thread a row, 521 so; 37 tokens: 13.8 and 12.3).
+    // tokens, f32, weights not lifted: 527 us with a step at a time and a thread a row, 521 so; 37 tokens: 13.8 and 12.3).
     constexpr int kSKeys = kTiles == 2 ? kStep : 2 * kStep;
     constexpr uint32_t kOCol = kTiles * kSBufs * kStep, kOCols = kSplit ? 2 * D : kSlim ? D : 128, kTmemCols = kSlim ? 256 : 512;
     constexpr uint32_t kPCol = kSlim ? kStep / 2 : 0;  // P lies this far into S
@@ -236,7 +236,10 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
     int seq, unit, n_new, first_token, len;
     if (b.n_seqs <= 32) {
         // A sequence per lane, every warp for itself: the target-th unit in order of key tiles, most first, so that
-        // the last CTAs are the shortest of the whole batch.
+        // the last CTAs are the shortest of the whole batch (f16, 64 columns, 7 heads to a kv head: 9 prompts up to 2500
+        // tokens 123 us, in batch order 133; 32 up to 1000 106 and 115; f32, 128 columns, 8 heads to each of 2 kv
+        // heads: 32 up to 1000 209 both ways, 32 up to 300 76 and 72).  Larger batches are taken in their own
+        // order: CTAs are many enough (64 up to 1000 tokens: 207 us and 416, twice the 32's).
         int t0 = 0, n = 0, l = 0;
         if (lane < b.n_seqs) {
             l = checked_len(b.lens[lane], b, b.status);
