@@ -502,14 +502,15 @@ attn_decode_kernel(const DecodeArgs p, const __grid_constant__ CUtensorMap kmap,
                     for (int i = 1; i < 8; ++i) mx = fmaxf(mx, z[r][i]);
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 1));
                     mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 2));
-                    const float mn = fmaxf(m[r], mx * sl[r]);
+                    const float mn = fmaxf(m[r], __fmul_rn(mx, sl[r]));
                     const float base = mn == -INFINITY ? 0.f : mn;
                     alpha[r] = ex2(m[r] - base);
                     m[r] = mn;
                     float sum = 0.f;
 #pragma unroll
                     for (int i = 0; i < 8; ++i) {
-                        z[r][i] = ex2(fmaf(z[r][i], sl[r], -base)) * kLift;
+                        // the product rounded as the maximum's was: what is left of the largest is 0 at any size
+                        z[r][i] = ex2(__fsub_rn(__fmul_rn(z[r][i], sl[r]), base)) * kLift;
                         sum += z[r][i];
                     }
                     l[r] = fmaf(l[r], alpha[r], sum);
