@@ -64,8 +64,8 @@ constexpr int kPart = 8;
 //   20 below                  8.7e-1   5.8e-4  2.2e-5  6.5e-6  5.0e-6
 //   f32 queries, D = 128      528 us   532     545     578     603
 //   f16 queries, D = 64       133 us   134     135     139     143     (packed ragged prompts)
-// f16 results have 11 bits and gain nothing from more than 2^11 (20 below: 4.7e-4 with 2^11 and 2^14).  bf16 has
-// f32's range.
+// (An operation more for each weight, where they are computed, has since made them 583 and 139.)  f16 results have 11
+// bits and gain nothing from more than 2^11 (20 below: 4.7e-4 with 2^11 and 2^14).  bf16 has f32's range.
 template <typename A, typename C> constexpr float kLift = std::is_same<C, __half>::value ? sizeof(A) == 4 ? 13.f : 11.f : 0.f;
 template <typename A, typename C> constexpr float kRescaleAt = std::is_same<C, __half>::value ? 15.f - kLift<A, C> : 8.f;
 struct PromptArgs {
@@ -76,6 +76,7 @@ struct PromptArgs {
     int unit_rows;       // rows of a CTA: two tiles, or one where that leaves at least half of the SMs idle
     int layer_row;
     int box_rows;  // rows per TMA box: page_size
+    float zero;    // 0
 };
 
 struct Shared {  // behind Q and the ring
@@ -646,8 +647,8 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
                 if (!(ok = other(mz, &theirs))) break;
                 mz = fmaxf(mz, theirs);
             }
-            const float m_new = fmaxf(m, mz * sl);
-            const bool grown = __any_sync(0xffffffffu, m_new > m + kRescaleAt<A, C>), part_end = kSplit && i0 > 0 && i0 % kPart == 0;
+            const float m_new = fmaxf(m, __fmul_rn(mz, sl));
+            const bool grown = __any_sync(0xffffffffu, m_new - m > kRescaleAt<A, C>), part_end = kSplit && i0 > 0 && i0 % kPart == 0;
             if (grown || part_end) {
                 float f = 1.f;
                 if (grown) {
@@ -686,7 +687,13 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
             }
             const float base = m == -INFINITY ? 0.f : m;
             float2 sum[2] = {both(0.f), both(0.f)};
-            const float2 sl2 = both(sl), nb2 = both(kLift<A, C> - base);
+            // An f16 weight keeps within the type however large the scores: their products with the scale are rounded as the
+            // maximum's was (from 2^24 on the exact product is units away from it), and a factor that next to the maximum
+            // rounds up is left out.  Product and sum are two operations (f16, 64 columns: 139 us, 136 as one; f32, 128
+            // columns: 583, 578); the product as one with a 0 that the compiler does not know, or it would join them.
+            float nb = kLift<A, C> - base;
+            if (kHalfType && nb + base > kLift<A, C>) nb = -base;
+            const float2 sl2 = both(sl), nb2 = both(nb), zero2 = both(p.zero);
 #pragma unroll
             for (int c0 = kStep - kHeld; c0 >= 0; c0 -= kHeld) {
                 if (c0 + kHeld < kStep) take(c0);
@@ -695,7 +702,8 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
                     uint32_t hi[16], lo[16];
 #pragma unroll
                     for (int k = 0; k < 16; ++k) {
-                        float2 x = fma2(make_float2(z[c + 2 * k], z[c + 2 * k + 1]), sl2, nb2);
+                        float2 x = make_float2(z[c + 2 * k], z[c + 2 * k + 1]);
+                        x = kHalfType ? add2(fma2(x, sl2, zero2), nb2) : fma2(x, sl2, nb2);
                         x = make_float2(ex2(x.x), !kSplit && k % 8 == 0 ? ex2_poly(x.y) : ex2(x.y));
                         sum[k & 1] = add2(sum[k & 1], x);
                         hi[k] = pack2<C>(x.x, x.y);
@@ -818,6 +826,7 @@ void launch_attn_prompt(const KvBatch& b, int act, const KvCache& kv, uint32_t l
     p.unit_rows = (act == MOE_T_F32 && b.head_dim == 128) || 2 * units_of(b, a, p.group, 2 * kRowTile) <= sm_count ? kRowTile : 2 * kRowTile;
     p.layer_row = static_cast<int>(static_cast<uint64_t>(layer) * kv.spec.n_pages * kv.spec.n_kv_heads * kv.spec.page_size);
     p.box_rows = static_cast<int>(kv.spec.page_size);
+    p.zero = 0.f;
     const CUtensorMap &k = kv.maps[2], &v = kv.maps[3];
     if (act == MOE_T_F32) {
         if (kv.spec.type == MOE_T_F16) launch_d<float, __half>(p, k, v, s);

@@ -16,7 +16,7 @@ def ctx():
     c.close()
 
 
-@pytest.mark.parametrize("kind", ["decode"])
+@pytest.mark.parametrize("kind", ["prompt", "decode"])
 @pytest.mark.parametrize("act,cache", [("f32", "f16"), ("f32", "bf16"), ("f16", "f16"), ("bf16", "bf16")])
 @pytest.mark.parametrize("dim", [64, 128])
 @pytest.mark.parametrize("heads", [2, 12])
