@@ -365,6 +365,7 @@ int moe_silu_mul(moe_ctx* ctx, uint64_t g_off, uint64_t u_off, uint64_t y_off, u
  * queries a prompt's weights are one piece (11 bits f16, 8 bf16: errors of the size of the outputs' own rounding).
  * With an f16 cache, whose smallest step is fixed, small weights have fewer bits: beside the above a weight is off by
  * up to 2^-36 (prompt, f16 queries), 2^-38 (prompt, f32) or 2^-40 (decode) of its row's largest.
+ * In a prompt over a bf16 cache scores have to be below 2^30 in magnitude (else a row can be NaN).
  * NaN and infinity: a row whose query or whose visible keys give a NaN score is NaN.  An infinite or NaN value makes its
  * column not finite in the rows that see it, NaN where the definition may be infinite (a weight's second piece
  * times infinity is NaN), and touches no other row. */

@@ -238,9 +238,9 @@ attn_prompt_kernel(const PromptArgs p, const __grid_constant__ CUtensorMap kmap,
     if (b.n_seqs <= 32) {
         // A sequence per lane, every warp for itself: the target-th unit in order of key tiles, most first, so that
         // the last CTAs are the shortest of the whole batch (f16, 64 columns, 7 heads to a kv head: 9 prompts up to 2500
-        // tokens 123 us, in batch order 133; 32 up to 1000 106 and 115; f32, 128 columns, 8 heads to each of 2 kv
-        // heads: 32 up to 1000 209 both ways, 32 up to 300 76 and 72).  Larger batches are taken in their own
-        // order: CTAs are many enough (64 up to 1000 tokens: 207 us and 416, twice the 32's).
+        // tokens 129 us, in batch order 137; 32 up to 1000 111 and 119; f32, 128 columns, 8 heads to each of 2 kv
+        // heads: 32 up to 1000 211 both ways, 32 up to 300 78 and 72).  Larger batches are taken in their own
+        // order: CTAs are many enough (64 up to 1000 tokens: 213 us and 420, twice the 32's).
         int t0 = 0, n = 0, l = 0;
         if (lane < b.n_seqs) {
             l = checked_len(b.lens[lane], b, b.status);
